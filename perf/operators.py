@@ -31,13 +31,13 @@ LISTED = [
     # SwiGLU hidden of the ~1B shape, odd number of rows
     {"name": "swiglu_8191x5632", "op": "quant", "T": 8191, "d": 5632, "swiglu": True},
     # q/k/v projection for one sequence of 32: weights from memory, latency
-    {"name": "linear_32x2304x768", "op": "linear", "M": 32, "N": 2304, "K": 768},
+    {"name": "linear_32x2304x768", "op": "linear", "M": 32, "N": 2304, "K": 768, "out": "bf16"},
     # q/k/v projection for 2048 tokens of the default model
-    {"name": "linear_2048x2304x768", "op": "linear", "M": 2048, "N": 2304, "K": 768},
-    # vocabulary projection of the masked rows of a batch: rows and columns ragged
-    {"name": "linear_777x30522x768", "op": "linear", "M": 777, "N": 30522, "K": 768},
+    {"name": "linear_2048x2304x768", "op": "linear", "M": 2048, "N": 2304, "K": 768, "out": "bf16"},
+    # vocabulary projection of the masked rows of a batch, fp32 logits, ragged in every direction
+    {"name": "linear_777x30522x768_f32", "op": "linear", "M": 777, "N": 30522, "K": 768, "out": "f32"},
     # gate/up projection of the ~1B shape at 16k tokens: matrix rate
-    {"name": "linear_16384x11264x2048", "op": "linear", "M": 16384, "N": 11264, "K": 2048},
+    {"name": "linear_16384x11264x2048", "op": "linear", "M": 16384, "N": 11264, "K": 2048, "out": "bf16"},
     # one step of sample() at its defaults: every position of one sequence, nucleus choice
     {"name": "sample_32x30522", "op": "sample", "T": 32, "V": 30522, "dtype": "bf16", "temperature": 1.0,
      "top_k": 0, "top_p": 0.9, "min_p": 0.0, "ids": True},
@@ -66,7 +66,8 @@ def draw(rng):
     if op == "quant":
         return {"op": op, "T": _log(rng, 1, 8191), "d": _log(rng, 24, 5632), "swiglu": rng.random() < 0.6}
     if op == "linear":
-        return {"op": op, "M": _log(rng, 1, 16384), "N": _log(rng, 16, 11264), "K": _log(rng, 32, 2048)}
+        m, n, k = _log(rng, 1, 16384), _log(rng, 16, 11264), _log(rng, 32, 2048)
+        return {"op": op, "M": m, "N": n, "K": k, "out": rng.choice(["bf16", "bf16", "f32"])}
     t = _log(rng, 1, 4096)
     v = _log(rng, 2, min(126464, (4096 * 30522) // t))
     return {"op": op, "T": t, "V": v, "dtype": rng.choice(["bf16", "f32"]),
@@ -88,7 +89,7 @@ def work(case):
                 "flops": n * (8 if case["swiglu"] else 2)}
     if op == "linear":
         m, n, k = case["M"], case["N"], case["K"]
-        return {"bytes": m * k + n * k + 2 * m * n + 4 * n, "flops": 2 * m * n * k}
+        return {"bytes": m * k + n * k + m * n * (4 if case["out"] == "f32" else 2) + 4 * n, "flops": 2 * m * n * k}
     # with ids about half of the positions are masked, and only their rows are wanted
     rows = case["T"] * (0.5 if case["ids"] else 1.0)
     return {"bytes": rows * case["V"] * (4 if case["dtype"] == "f32" else 2) + 20 * case["T"],
@@ -211,7 +212,7 @@ def _widen(q, scale, rows):
 
 def _plain_linear(s):
     y = torch.matmul(_widen(s["xq"], s["xs"], 1), _widen(s["wq"], s["ws"], BLOCK).t()) + s["bias"]
-    return y.to(torch.bfloat16)
+    return y if s["case"]["out"] == "f32" else y.to(torch.bfloat16)
 
 
 def _plain_sample(s):
@@ -248,7 +249,8 @@ def _own(s):
         q, scale = ops.quantize_fp8(s["x"], "swiglu" if c["swiglu"] else None)
         return {"q": q, "scale": scale}
     if c["op"] == "linear":
-        return ops.fp8_matmul(s["xq"], s["xs"], s["wq"], s["ws"], bias=s["bias"])
+        return ops.fp8_matmul(s["xq"], s["xs"], s["wq"], s["ws"], bias=s["bias"],
+                              out_dtype=torch.float32 if c["out"] == "f32" else torch.bfloat16)
     return ops.sample_tokens(s["logits"], s["u"], temperature=c["temperature"], top_k=c["top_k"], top_p=c["top_p"],
                              min_p=c["min_p"], ids=s["ids"], mask_token_id=s["mask_id"])
 
