@@ -330,6 +330,11 @@ int ldm_quant_fp8_block(const float *w, int64_t ld_w, int64_t N, int64_t K, uint
 int ldm_gemm_fp8(int64_t M, int64_t N, int64_t K, const uint8_t *A, int64_t lda, const uint8_t *sA, int64_t ld_sa,
                  const uint8_t *B, int64_t ldb, const uint8_t *sB, int64_t ld_sb, const float *bias, void *C,
                  int64_t ldc, void *stream);
+/* The same product with C fp32 (4-byte aligned): every product of two e4m3 values is kept whole (bf16 MFMA), each 32
+ * positions are added within 2^-22 of the sum of their magnitudes. */
+int ldm_gemm_fp8_f32(int64_t M, int64_t N, int64_t K, const uint8_t *A, int64_t lda, const uint8_t *sA, int64_t ld_sa,
+                     const uint8_t *B, int64_t ldb, const uint8_t *sB, int64_t ld_sb, const float *bias, float *C,
+                     int64_t ldc, void *stream);
 
 /* ---------------------------------------------------------------- K4: masked cross-entropy
  * masked_cross_entropy_loss / variational_lower_bound_loss (src/loss.py:8-65).

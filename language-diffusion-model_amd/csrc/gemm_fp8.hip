@@ -1,13 +1,18 @@
 // 8-bit matrix product of the inference projections on the scaled MFMA of gfx950:
 //   C[m, n] = sum_kb 2^(ea[m, kb] + eb[n / 128, kb]) * sum_{k in block kb} A[m, k] * B[n, k]  (+ bias[n])
 // A [M, K] e4m3 rows with one E8M0 scale per 128 columns, B [N, K] e4m3 weights with one per 128 x 128 block, fp32
-// accumulation, bf16 output.  v_mfma_scale_f32_16x16x128_f8f6f4 takes an E8M0 scale per row and 32 values of
-// either operand: power-of-two scales cost no vector instruction, where a general fp32 scale would need one
-// multiply-add per accumulator and block beside the matrix pipe (about half its time again).
+// accumulation, bf16 or fp32 output.
 //
-// Precision, measured: of the eight products of a lane's consecutive K positions each is truncated at 2^-13 of the leading
-// bit of the largest; the groups of eight are added in fp32.  Random operands lose 1.5e-5 of the result (2-norm), well
-// below the bf16 rounding of the output (1.7e-3); an fp32 output would not be one, so there is none.
+// bf16 output: v_mfma_scale_f32_16x16x128_f8f6f4 takes an E8M0 scale per row and 32 values of either operand: power-of-two
+// scales cost no vector instruction, where a general fp32 scale would need one multiply-add per accumulator and block
+// beside the matrix pipe (about half its time again).  Precision, measured: of the eight products of a lane's consecutive
+// K positions each is truncated at 2^-13 of the leading bit of the largest; the groups of eight are added in fp32.  Random
+// operands lose 1.5e-5 of the result (2-norm), well below the bf16 rounding of the output (1.7e-3), but far above fp32's.
+//
+// fp32 output: the unscaled 8-bit MFMA truncates likewise, the bf16 one does not (one product of 32 positions of e4m3 values
+// is within 2^-22 of the sum of their magnitudes, 5e-8 in the 2-norm).  e4m3 values are bf16 values, so the fragments are
+// widened in registers and four 16x16x32 bf16 MFMAs form a block's sum, which ldexp scales into the accumulator: half the
+// matrix rate, and two vector instructions per accumulator and block.
 #include <type_traits>
 
 #include "fp8.h"
@@ -26,7 +31,7 @@ struct GArgs {
   const uint8_t *B; int64_t ldb;
   const uint8_t *sB; int64_t ld_sb;
   const float *bias;
-  bf16_t *C; int64_t ldc;
+  void *C; int64_t ldc;
 };
 
 __device__ __forceinline__ f4v mfma_scaled(const i8v &a, const i8v &b, const f4v &c, int sa, int sb) {
@@ -52,10 +57,63 @@ __device__ __forceinline__ i8v join(const i4v &a, const i4v &b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// fp32 output: a fragment's 32 values as four bf16 operands (positions 8 s .. 8 s + 7 of the lane's 32 in operand s, of either
+// side alike)
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+struct Wide { b8v s[4]; };
+__device__ __forceinline__ Wide widen(const i8v &x) {
+  Wide w;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    i4v d;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const b2v lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[2 * s + h], 1.0f, false);
+      const b2v hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[2 * s + h], 1.0f, true);
+      d[2 * h] = __builtin_bit_cast(int, lo);
+      d[2 * h + 1] = __builtin_bit_cast(int, hi);
+    }
+    w.s[s] = __builtin_bit_cast(b8v, d);
+  }
+  return w;
+}
+// acc[j] += 2^(ea + eb) * (b[j] . a), from the scales' codes (255 is NaN).  ldexp, for the power itself may lie outside fp32
+// where the result does not.
+template <int TN>
+__device__ __forceinline__ void add_block(f4v (&acc)[TN], const Wide (&b)[TN], const Wide &a, int ea, int eb) {
+  const float c0 = ea == 255 || eb == 255 ? __builtin_nanf("") : 0.f;
+  const int e = ea + eb - 254;
+  f4v p[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) p[j] = f4v{c0, c0, c0, c0};
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) p[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].s[s], a.s[s], p[j], 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[j][k] += ldexpf(p[j][k], e);
+}
+// one 16 x 16 block of outputs, either way
+template <typename OT>
+__device__ __forceinline__ void add_one(f4v &acc, const i8v &b, const i8v &a, int ea, int eb) {
+  if constexpr (std::is_same_v<OT, float>) {
+    f4v t[1] = {acc};
+    const Wide w[1] = {widen(b)};
+    add_block(t, w, widen(a), ea, eb);
+    acc = t[0];
+  } else {
+    acc = mfma_scaled(b, a, acc, eb, ea);
+  }
+}
+
 // four consecutive columns of a row of C
+template <typename OT>
 __device__ __forceinline__ void store4(const GArgs &g, int64_t m, int64_t n, f4v v, bool vec) {
   if (m >= g.M || n >= g.N) return;
-  bf16_t *c = g.C + m * g.ldc + n;
+  OT *c = (OT *)g.C + m * g.ldc + n;
   if (n + 4 <= g.N) {
     if (g.bias) {
 #pragma unroll
@@ -65,19 +123,19 @@ __device__ __forceinline__ void store4(const GArgs &g, int64_t m, int64_t n, f4v
       st4(c, f4{{v[0], v[1], v[2], v[3]}});
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Elt<bf16_t>::st(c + j, v[j]);
+      for (int j = 0; j < 4; ++j) Elt<OT>::st(c + j, v[j]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (n + j < g.N) Elt<bf16_t>::st(c + j, v[j] + (g.bias ? g.bias[n + j] : 0.f));
+      if (n + j < g.N) Elt<OT>::st(c + j, v[j] + (g.bias ? g.bias[n + j] : 0.f));
   }
 }
 
 // Few rows: the weights are the traffic.  A workgroup owns 16 columns and 16 * MT rows, its four waves split the
 // blocks of K and add up through LDS; fragments come straight from memory (a 16 x 128-byte fragment is 16 whole lines).
 // The weights are the FIRST operand, so a lane ends up with four consecutive columns of one row.
-template <int MT>
+template <int MT, typename OT>
 __global__ __launch_bounds__(256) void gemm_fp8_rows_k(GArgs g, bool vec) {
   __shared__ f4v red[4][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -105,7 +163,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_rows_k(GArgs g, bool vec) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const i8v fa = join(*reinterpret_cast<const i4v *>(a[i] + k), *reinterpret_cast<const i4v *>(a[i] + k + 16));
-      acc[i] = mfma_scaled(fb, fa, acc[i], eb, sa[i][kb]);
+      add_one<OT>(acc[i], fb, fa, sa[i][kb], eb);
     }
   }
   if (kb < nkb) {
@@ -115,7 +173,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_rows_k(GArgs g, bool vec) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const i8v fa = join(load16_tail(a[i], k, g.K), load16_tail(a[i], k + 16, g.K));
-      acc[i] = mfma_scaled(fb, fa, acc[i], eb, sa[i][kb]);
+      add_one<OT>(acc[i], fb, fa, sa[i][kb], eb);
     }
   }
 #pragma unroll
@@ -124,7 +182,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_rows_k(GArgs g, bool vec) {
   for (int t = threadIdx.x; t < MT * 64; t += 256) {
     const int i = t >> 6, l = t & 63;
     const f4v v = (red[0][i][l] + red[1][i][l]) + (red[2][i][l] + red[3][i][l]);
-    store4(g, m0 + i * 16 + (l & 15), n0 + (l >> 4) * 4, v, vec);
+    store4<OT>(g, m0 + i * 16 + (l & 15), n0 + (l >> 4) * 4, v, vec);
   }
 }
 
@@ -150,7 +208,7 @@ __device__ __forceinline__ void lds_dma16(unsigned lds, unsigned off, const uint
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 
-template <int TM>
+template <int TM, typename OT>
 __global__ __launch_bounds__(256, 2) void gemm_fp8_tile_k(GArgs g, int tiles_m, int tiles_n, int band, bool vec) {
   constexpr int BM = 32 * TM, BN = FP8_BLOCK, TN = 4;
   constexpr int STAGE = (BM + BN) * FP8_BLOCK;
@@ -263,6 +321,15 @@ __global__ __launch_bounds__(256, 2) void gemm_fp8_tile_k(GArgs g, int tiles_m, 
     i8v fb[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[j] = frag(sb + j * (4 * FP8_BLOCK), rdB);
+    if constexpr (std::is_same_v<OT, float>) {
+      Wide wb[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) wb[j] = widen(fb[j]);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        add_block(acc[i], wb, widen(frag(sa + i * (16 * FP8_BLOCK), rdA)), (ea[i / 4] >> (8 * (i % 4))) & 255, eb);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const i8v fa = frag(sa + i * (16 * FP8_BLOCK), rdA);
@@ -296,6 +363,33 @@ __global__ __launch_bounds__(256, 2) void gemm_fp8_tile_k(GArgs g, int tiles_m, 
         bv[j][e] = b[c < left ? c : left - 1];
       }
   }
+  if constexpr (std::is_same_v<OT, float>) {      // (fp32: 64 bytes of one row per lane as it is, the transposition alone)
+    const int64_t c = n0 + wn * (16 * TN) + q * 16 + (lane & 3) * 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      unsigned p[4][4];      // [element][piece of 4 columns]
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e][j] = __float_as_uint(acc[i][j][e] + bv[j][e]);
+      quad_transpose4(p);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int64_t m = m0 + wm * (16 * TM) + i * 16 + ((lane >> 2) & 3) * 4 + t;
+        if (m < g.M && c < g.N) {
+          unsigned *o = (unsigned *)g.C + m * g.ldc + c;
+          if (vec && c + 4 <= g.N) {
+            *reinterpret_cast<uint4 *>(o) = make_uint4(p[0][t], p[1][t], p[2][t], p[3][t]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < g.N) o[e] = p[e][t];
+          }
+        }
+      }
+    }
+    return;
+  }
   const int64_t c = n0 + wn * (16 * TN) + (q >> 1) * 32 + (lane & 3) * 8;
 #pragma unroll
   for (int i = 0; i < TM; i += 2) {
@@ -315,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void gemm_fp8_tile_k(GArgs g, int tiles_m, 
     for (int t = 0; t < 4; ++t) {
       const int64_t m = m0 + wm * (16 * TM) + (i + (q & 1)) * 16 + ((lane >> 2) & 3) * 4 + t;
       if (m < g.M && c < g.N) {
-        bf16_t *o = g.C + m * g.ldc + c;
+        bf16_t *o = (bf16_t *)g.C + m * g.ldc + c;
         if (vec && c + 8 <= g.N) {
           *reinterpret_cast<uint4 *>(o) = make_uint4(p[0][t], p[1][t], p[2][t], p[3][t]);
         } else if (vec) {      // (pairs: single elements cost 1000x1111x1000 4 %)
@@ -334,35 +428,36 @@ __global__ __launch_bounds__(256, 2) void gemm_fp8_tile_k(GArgs g, int tiles_m, 
   }
 }
 
-template <int TM>
+template <int TM, typename OT>
 int launch_tile(const GArgs &g, hipStream_t s) {
   constexpr int BM = 32 * TM, LDS = 2 * (BM + 128) * FP8_BLOCK + SCH * (BM + 1);
   const int64_t tm = ceil_div(g.M, BM), tn = ceil_div(g.N, 128);
   if (tm > 0x3fffffff || tn > 0x3fffffff || tm * tn > 0x3fffffff) return LDM_E_SHAPE;
   // 32-bit source offsets inside a tile
   if (g.lda >= (1 << 23) || g.ldb >= (1 << 23)) return LDM_E_SHAPE;
-  const bool vec = g.ldc % 8 == 0 && aligned_to(g.C, 16);
+  const bool vec = g.ldc % (16 / (int)sizeof(OT)) == 0 && aligned_to(g.C, 16);
   static std::atomic<uint64_t> attr_done{0};
   uint64_t bit;
   if (ldm_attr_pending(attr_done, &bit)) {
-    (void)hipFuncSetAttribute((const void *)gemm_fp8_tile_k<TM>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    (void)hipFuncSetAttribute((const void *)gemm_fp8_tile_k<TM, OT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     attr_done.fetch_or(bit, std::memory_order_release);
   }
-  hipLaunchKernelGGL(gemm_fp8_tile_k<TM>, dim3((unsigned)(tm * tn)), dim3(256), LDS, s, g, (int)tm, (int)tn, 8, vec);
+  hipLaunchKernelGGL((gemm_fp8_tile_k<TM, OT>), dim3((unsigned)(tm * tn)), dim3(256), LDS, s, g, (int)tm, (int)tn, 8, vec);
   LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
 
+template <typename OT>
 int launch_rows(const GArgs &g, hipStream_t s) {
-  const bool vec = g.ldc % 4 == 0 && aligned_to(g.C, 8);
+  const bool vec = g.ldc % 4 == 0 && aligned_to(g.C, 4 * sizeof(OT));
   const int64_t gx = ceil_div(g.N, 16);
   const int mt = g.M <= 16 ? 1 : g.M <= 32 ? 2 : 4;
   const int64_t gy = ceil_div(g.M, 16 * mt);
   if (gx > 0x7fffffff || gy > 65535) return LDM_E_SHAPE;
   const dim3 grid((unsigned)gx, (unsigned)gy), wg(256);
-  if (mt == 1) hipLaunchKernelGGL((gemm_fp8_rows_k<1>), grid, wg, 0, s, g, vec);
-  else if (mt == 2) hipLaunchKernelGGL((gemm_fp8_rows_k<2>), grid, wg, 0, s, g, vec);
-  else hipLaunchKernelGGL((gemm_fp8_rows_k<4>), grid, wg, 0, s, g, vec);
+  if (mt == 1) hipLaunchKernelGGL((gemm_fp8_rows_k<1, OT>), grid, wg, 0, s, g, vec);
+  else if (mt == 2) hipLaunchKernelGGL((gemm_fp8_rows_k<2, OT>), grid, wg, 0, s, g, vec);
+  else hipLaunchKernelGGL((gemm_fp8_rows_k<4, OT>), grid, wg, 0, s, g, vec);
   LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
@@ -377,19 +472,20 @@ constexpr int64_t CUS = 256;
 // more rounds (us at 64 / 128 rows: 2048x2304x768, one round each, 9.9 / 10.1; 2048x768x768 5.6 / 7.5; 4096x2304x768, two each,
 // 15.4 / 16.7; 8192x2304x768, three each, 25.7 / 25.7; 3000x2304x768, two against one, 14.5 / 11.1; 256x30522x768 15.1 / 12.8;
 // 512x30522x768, three against two, 23.7 / 22.3; 777x30522x768 34.5 / 33.5; 4096x2048x2048 26.8 / 19.6).
+template <typename OT>
 int launch_tiles(const GArgs &g, hipStream_t s) {
   const int64_t tn = ceil_div(g.N, 128);
   const bool low = ceil_div(ceil_div(g.M, 64) * tn, 3 * CUS) <= ceil_div(ceil_div(g.M, 128) * tn, 2 * CUS);
-  const int rc = low ? launch_tile<2>(g, s) : launch_tile<4>(g, s);
-  return rc == LDM_E_SHAPE ? launch_rows(g, s) : rc;      // (row strides of 8 MiB and more)
+  const int rc = low ? launch_tile<2, OT>(g, s) : launch_tile<4, OT>(g, s);
+  return rc == LDM_E_SHAPE ? launch_rows<OT>(g, s) : rc;      // (row strides of 8 MiB and more)
 }
 
-GArgs columns_from(const GArgs &g, int64_t n) {      // n: a multiple of 128
+GArgs columns_from(const GArgs &g, int64_t n) {      // bf16 output; n: a multiple of 128
   GArgs t = g;
   t.N = g.N - n;
   t.B += n * g.ldb;
   t.sB += n / FP8_BLOCK * g.ld_sb;
-  t.C += n;
+  t.C = (bf16_t *)g.C + n;
   if (t.bias) t.bias += n;
   return t;
 }
@@ -403,18 +499,40 @@ GArgs columns_from(const GArgs &g, int64_t n) {      // n: a multiple of 128
 //     18.0 / 17.8; 15001x2304x768: 0.69 of 3 44.5 / 41.8; 8192x2304x768: 0.56 of 2 28.8 / 25.7; 4096x11264x2048: 0.92 of 3
 //     88 / 119).  Columns behind the last multiple of 128 are a second launch: it pays where the first one saves more
 //     (1024x30522x768: 0.93 of 2 44.3 / 46.0; 15001x11200x768: 0.91 of 11 184 / 186).
+//   fp32 output has rows and tiles: rows up to two workgroups per CU (64 x 128 tiles: 96x2304x768 5.9 / 8.7, 512x768x768 6.6 /
+//     8.7, 64x11264x2048 18.5 / 16.8, 2048x768x768 16.7 / 9.3; up to 32 rows 32x11264x2048 11.4 / 16.2, 32x30522x768 11.9 / 8.8;
+//     16x30522x768 8.0 / 8.1), and the same choice of tile height (64 / 128 rows: 2048x2304x768 17.0 / 20.1, 3000x2304x768 21.9 /
+//     20.5, 8192x2304x768 43.5 / 43.7, 512x30522x768 39.0 / 36.5, 777x30522x768 59.0 / 58.2).  16384x11264x2048 768 us = 985
+//     TFLOP/s: by instruction count a block's 64 bf16 MFMAs (1024 cycles a wave) have 512 cycles of ldexp and additions and
+//     512 of widening beside them, and MFMAs and vector instructions of a SIMD's waves do not overlap on this card.
+template <typename OT>
 int launch(const GArgs &g, hipStream_t s) {
   const int64_t gx = ceil_div(g.N, 16);
-  if (g.M <= 16 || gx * ceil_div(g.M, 64) <= (g.M <= 32 ? 4 * CUS : CUS)) return launch_rows(g, s);
+  constexpr int64_t FEW = std::is_same_v<OT, float> ? 2 * CUS : CUS;
+  if (g.M <= 16 || gx * ceil_div(g.M, 64) <= (g.M <= 32 ? 4 * CUS : FEW)) return launch_rows<OT>(g, s);
+  if constexpr (std::is_same_v<OT, float>) return launch_tiles<OT>(g, s);
   const int64_t n128 = g.N / FP8_BLOCK * FP8_BLOCK;
   const int64_t rounds = ceil_div(ceil_div(g.M, 256) * ceil_div(n128, 256), CUS);
   if ((double)g.M * (double)n128 >= (n128 == g.N ? 0.75 : 0.85) * 65536.0 * (double)(rounds * CUS)) {
     GArgs m = g;
     m.N = n128;
     const int rc = launch_4w(m, s);
-    if (rc != LDM_E_SHAPE && rc != LDM_E_ALIGN) return rc != LDM_OK || n128 == g.N ? rc : launch_tiles(columns_from(g, n128), s);
+    if (rc != LDM_E_SHAPE && rc != LDM_E_ALIGN) return rc != LDM_OK || n128 == g.N ? rc : launch_tiles<OT>(columns_from(g, n128), s);
   }
-  return launch_tiles(g, s);
+  return launch_tiles<OT>(g, s);
+}
+
+// checks of the C entries; elt: bytes of an output element
+int checked(const GArgs &g, int elt) {
+  if (g.M < 0 || g.N < 0 || g.K <= 0) return LDM_E_BADARG;
+  if (g.M == 0 || g.N == 0) return LDM_OK;
+  if (!g.A || !g.sA || !g.B || !g.sB || !g.C) return LDM_E_BADARG;
+  const int64_t kb = ceil_div(g.K, FP8_BLOCK);
+  if (g.lda < g.K || g.ldb < g.K || g.ldc < g.N || g.ld_sa < kb || g.ld_sb < kb) return LDM_E_BADARG;
+  if (g.lda % 16 || g.ldb % 16 || !aligned_to(g.A, 16) || !aligned_to(g.B, 16)) return LDM_E_ALIGN;
+  if (!aligned_to(g.C, elt) || (g.bias && !aligned_to(g.bias, 4))) return LDM_E_ALIGN;
+  if (g.M > (1ll << 40) || g.N > (1ll << 31) || g.K > (1 << 28)) return LDM_E_SHAPE;
+  return LDM_OK;
 }
 
 }  // namespace
@@ -422,15 +540,15 @@ int launch(const GArgs &g, hipStream_t s) {
 extern "C" int ldm_gemm_fp8(int64_t M, int64_t N, int64_t K, const uint8_t *A, int64_t lda, const uint8_t *sA,
                             int64_t ld_sa, const uint8_t *B, int64_t ldb, const uint8_t *sB, int64_t ld_sb,
                             const float *bias, void *C, int64_t ldc, void *stream) {
-  if (M < 0 || N < 0 || K <= 0) return LDM_E_BADARG;
-  if (M == 0 || N == 0) return LDM_OK;
-  if (!A || !sA || !B || !sB || !C) return LDM_E_BADARG;
-  const int64_t kb = ceil_div(K, FP8_BLOCK);
-  if (lda < K || ldb < K || ldc < N || ld_sa < kb || ld_sb < kb) return LDM_E_BADARG;
-  if (lda % 16 || ldb % 16 || !aligned_to(A, 16) || !aligned_to(B, 16)) return LDM_E_ALIGN;
-  if (!aligned_to(C, 2) || (bias && !aligned_to(bias, 4))) return LDM_E_ALIGN;
-  if (M > (1ll << 40) || N > (1ll << 31) || K > (1 << 28)) return LDM_E_SHAPE;
-  GArgs g{M, N, K, A, lda, sA, ld_sa, B, ldb, sB, ld_sb, bias, (bf16_t *)C, ldc};
-  hipStream_t s = (hipStream_t)stream;
-  return launch(g, s);
+  const GArgs g{M, N, K, A, lda, sA, ld_sa, B, ldb, sB, ld_sb, bias, C, ldc};
+  const int rc = checked(g, 2);
+  return rc != LDM_OK || M == 0 || N == 0 ? rc : launch<bf16_t>(g, (hipStream_t)stream);
+}
+
+extern "C" int ldm_gemm_fp8_f32(int64_t M, int64_t N, int64_t K, const uint8_t *A, int64_t lda, const uint8_t *sA,
+                                int64_t ld_sa, const uint8_t *B, int64_t ldb, const uint8_t *sB, int64_t ld_sb,
+                                const float *bias, float *C, int64_t ldc, void *stream) {
+  const GArgs g{M, N, K, A, lda, sA, ld_sa, B, ldb, sB, ld_sb, bias, C, ldc};
+  const int rc = checked(g, 4);
+  return rc != LDM_OK || M == 0 || N == 0 ? rc : launch<float>(g, (hipStream_t)stream);
 }

@@ -135,3 +135,24 @@ def test_filters_of_the_draw_are_checked_at_every_temperature(monkeypatch):
                             (0.0, dict(top_p=1.5)), (0.0, dict(min_p=-0.5)), (1.0, dict(top_p=0.0))):
         with pytest.raises(ValueError):
             DiffusionLanguageModel._pick_tokens(m, seq, logits, temperature, **kw)
+
+
+def test_fp32_product_refusals():
+    from src import _native as N
+    from src import ops
+    q = torch.zeros(4, 16).to(torch.float8_e4m3fn)
+    s = torch.zeros(4, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    for dt in (torch.float16, torch.float64, torch.int32, None):
+        with pytest.raises(TypeError, match="out_dtype"):
+            ops.fp8_matmul(q, s, q, s[:1], out_dtype=dt)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        ops.fp8_matmul(q, s, q, s[:1], out_dtype=torch.float32)
+    P = 4096      # an address that is never read
+
+    def gemm(M=4, n=8, K=256, A=P, lda=256, sA=P, lsa=2, B=P, ldb=256, sB=P, lsb=2, bias=None, C=P, ldc=8):
+        return N.lib().ldm_gemm_fp8_f32(M, n, K, A, lda, sA, lsa, B, ldb, sB, lsb, bias, C, ldc, None)
+    assert gemm(M=0) == 0 and gemm(n=0) == 0
+    assert gemm(K=0) == BADARG and gemm(M=-1) == BADARG and gemm(C=None) == BADARG and gemm(lda=240) == BADARG
+    assert gemm(ldc=7) == BADARG and gemm(lsa=1) == BADARG and gemm(lsb=1) == BADARG
+    assert gemm(lda=264) == ALIGN and gemm(B=P + 8) == ALIGN and gemm(C=P + 2) == ALIGN and gemm(bias=P + 2) == ALIGN
+    assert gemm(K=(1 << 28) + 1, lda=1 << 29, ldb=1 << 29, lsa=1 << 22, lsb=1 << 22) == SHAPE
