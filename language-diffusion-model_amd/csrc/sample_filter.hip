@@ -137,7 +137,7 @@ struct Row {
   float cf;          // log2(e) / temperature
   double dmx, c;     // mx; log2(e) / temperature
   int shift;
-  // round(2^shift * 2^-x), x = c (mx - l) >= 0 and at most about shift + 3 (logits are held to `floor`, where the weight is
+  // round(2^shift * 2^-x), x = c (mx - l) >= 0 and at most about 2 (shift + 3) (logits are held to `floor`, where the weight is
   // 0): 2^-n times a polynomial for 2^f on |f| <= 1/2 (degree 9 through the Chebyshev nodes, constant term 1: off by
   // 3e-14).  n comes out of adding 1.5 * 2^52, the power of two goes into the exponent bits, and the integer out of adding
   // 2^52: the conversions, roundings and scalings of doubles that the card has run at a quarter of the rate of these sums.
@@ -628,10 +628,12 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_k(const T *logits, FArg
     if (threadIdx.x == 0) a.out[r] = 0;
     return;
   }
-  // logits below it have weight 0 (ln 2 < 0.7); temperatures are within 1e-28 .. 1e28, so it is either finite and at least half
-  // a step of mx away, or mx itself
+  // Logits at and below it have weight 0 (ln 2 < 0.7): masked places and what lies behind the row stand there.  Where `vanish` is
+  // a few steps of mx the subtraction may round towards mx, and half a step leaves a weight: then the next lower float.
+  // Temperatures are within 1e-28 .. 1e28, so it is either finite and at least half a step of mx away, or mx itself
   const float vanish = (float)(0.7 * (a.shift + 3) / a.inv_temp);
-  const float floor = mx < INFINITY ? fmaxf(mx - vanish, -3.402823466e38f) : mx;
+  float floor = mx < INFINITY ? fmaxf(mx - vanish, -3.402823466e38f) : mx;
+  if (floor != mx && mx - floor < vanish) floor = fmaxf(nextafterf(floor, -INFINITY), -3.402823466e38f);
   if (floor == mx) {
     if (wid == 0) {
       const int tok = choose_equal(row, a, mx, a.u[r]);
