@@ -64,3 +64,53 @@ def test_temperatures_of_a_few_steps_of_the_largest_logit(dev, V, mx):
                 got = ops.sample_tokens(z.to(dev), ur.to(dev), temperature=T, **f).cpu()
                 assert int(got.max()) < V, (steps, u, f, got)
                 assert torch.equal(got, choose(z, ur, temperature=T, **f)), (steps, u, f)
+
+
+def agree(dev, z, u, copies=1, **f):
+    """The rows' tokens, with every row `copies` times (the number of rows decides which kernel runs)."""
+    from src import ops
+    got = ops.sample_tokens(z.to(dev).repeat(copies, 1), u.to(dev).repeat(copies), **f).cpu().view(copies, -1)
+    want = choose(z, u, **f)
+    assert bool((got == want).all()), (f, got[0], want)
+    return want
+
+
+@pytest.mark.parametrize("V,copies", [(1000, 1), (5000, 1), (9000, 1), (9000, 130), (9000, 260), (30522, 1)])
+def test_thousands_of_different_logits_in_one_bin(dev, V, copies):
+    """Nearly flat rows and one far lower finite logit: the bins span that distance, the second histogram's too."""
+    g = torch.Generator().manual_seed(V)
+    z = 1e-6 * torch.randn(4, V, generator=g)
+    z[:, 7] = -40.0
+    z[1, ::3] = z[1, 5]                           # a third of them equal, at an ordinary place
+    z[2] = torch.round(z[2] * 3e7) / 3e7          # every value many times
+    z[2, 7] = -1e5
+    z[3, : V // 2] = torch.sort(z[3, : V // 2]).values
+    z[3, 7] = -40.0
+    u = torch.rand(4, generator=g)
+    cluster = V - 1
+    for f in (dict(top_k=V // 2), dict(top_k=V // 3 + 1, temperature=0.5), dict(top_p=0.5), dict(top_p=0.3, temperature=1.7),
+              dict(top_k=2 * V // 3, top_p=0.5), dict(top_k=cluster, top_p=0.999), dict(top_p=0.7, min_p=0.5)):
+        for uu in (u, torch.full((4,), ONE), torch.zeros(4)):
+            agree(dev, z, uu, copies, **f)
+
+
+@pytest.mark.parametrize("V,copies", [(8192, 1), (9000, 1), (65000, 1), (65000, 260), (126464, 1), (126464, 130)])
+def test_mass_that_the_estimate_does_not_see(dev, V, copies):
+    """A tail of tokens that an estimate in units of 2^-32 rounds to nothing, and a top_p whose border lies in it."""
+    g = torch.Generator().manual_seed(V)
+    z = torch.empty(4, V)
+    low = 33.03 * math.log(2.0)                   # weight 2^-33.03 of the largest
+    z[0] = -low
+    z[1] = -low * (1 + 0.01 * torch.rand(V, generator=g))
+    z[2] = -low * (1 + 1e-6 * torch.rand(V, generator=g))
+    z[3] = -low * (1 + 0.2 * torch.rand(V, generator=g))
+    z[:, V // 5] = 0.0
+    tail = 2.0 ** -33.03 * V
+    moved = 0
+    for share in (0.3, 0.8):
+        # kept mass of the tail: about `share` of it (less where its weights differ)
+        top_p = (1 + share * tail) / (1 + tail)
+        for f in (dict(), dict(min_p=2.0 ** -33.5), dict(top_k=V - 3)):
+            for u in (1 - 2.0 ** -22, ONE, 0.5):
+                moved += int((agree(dev, z, torch.full((4,), u), copies, top_p=top_p, **f) != V // 5).sum())
+    assert moved > 0                              # (the tail was drawn from)
