@@ -1591,7 +1591,8 @@ class Fp8Weights:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("8-bit copies of changed (or not yet used) weights cannot be written while a graph is "
                                    "captured: run the call once before the capture")
-            with torch.no_grad():
+            # (copies made in inference mode could not be written again outside it)
+            with torch.inference_mode(False), torch.no_grad():
                 w = self.weights[0] if len(self.weights) == 1 else torch.cat([w.detach() for w in self.weights])
                 b = torch.cat([b.detach().float() for b in self.biases])
                 if self.q is not None and self.q.device == w.device:

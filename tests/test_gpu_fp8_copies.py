@@ -1,0 +1,24 @@
+"""The 8-bit copies of weights: modes, threads, replaced parameters, on a real MI355X."""
+import pytest
+import torch
+
+from test_gpu_fp8 import make_layer
+from test_gpu_fp8_model import batch, make
+
+pytestmark = pytest.mark.gpu
+
+
+def test_copies_made_in_inference_mode_are_written_again_outside_it(dev):
+    from src import ops
+    lin, packs = make_layer(dev)
+    x = torch.randn(5, 192, device=dev).bfloat16()
+    with torch.inference_mode():
+        y0 = ops.fp8_linear(x, packs[2])
+    with torch.no_grad():
+        lin[3].weight.mul_(2.0)
+        lin[3].bias.mul_(2.0)
+        assert torch.equal(ops.fp8_linear(x, packs[2]), 2 * y0)
+        lin[3].weight.mul_(2.0)
+        lin[3].bias.mul_(2.0)
+    with torch.inference_mode():          # and the other way round
+        assert torch.equal(ops.fp8_linear(x, packs[2]), 4 * y0)
