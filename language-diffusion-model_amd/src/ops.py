@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import math
 import os
+import threading
 
 import torch
 from torch import Tensor
@@ -1583,37 +1584,45 @@ class Fp8Weights:
         self.k = int(self.weights[0].shape[1])
         self._key = None
         self._written = self._stream = None      # event behind the last writing, and the stream it ran on
+        self._lock = threading.Lock()            # (one thread writes, the others find the copies and their event whole)
         self.q = self.scale = self.b = None
 
     def get(self):
         key = (WEIGHTS_EPOCH, SHADOW_GEN) + tuple((p._version, p.data_ptr()) for p in self.weights + self.biases)
-        if key != self._key:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("8-bit copies of changed (or not yet used) weights cannot be written while a graph is "
-                                   "captured: run the call once before the capture")
-            # (copies made in inference mode could not be written again outside it)
-            with torch.inference_mode(False), torch.no_grad():
-                w = self.weights[0] if len(self.weights) == 1 else torch.cat([w.detach() for w in self.weights])
-                b = torch.cat([b.detach().float() for b in self.biases])
-                if self.q is not None and self.q.device == w.device:
-                    self._wait(w.device)         # (an earlier writing on another stream)
-                    quantize_fp8_weight(w.detach(), out=(self.q, self.scale))
-                    self.b.copy_(b)
-                else:
-                    self.q, self.scale = quantize_fp8_weight(w.detach())
-                    self.b = b
-                stream = torch.cuda.current_stream(w.device)
-                self._written = torch.cuda.Event()
-                self._written.record(stream)
-                self._stream = stream.cuda_stream
-            self._key = key
-        else:
-            self._wait(self.q.device)
-        return self.q, self.scale, self.b
+        with self._lock:
+            if key != self._key:
+                self._write(key)
+            else:
+                self._wait(self.q.device)
+            return self.q, self.scale, self.b
+
+    def _write(self, key) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("8-bit copies of changed (or not yet used) weights cannot be written while a graph is "
+                               "captured: run the call once before the capture")
+        # (copies made in inference mode could not be written again outside it)
+        with torch.inference_mode(False), torch.no_grad():
+            w = self.weights[0] if len(self.weights) == 1 else torch.cat([w.detach() for w in self.weights])
+            b = torch.cat([b.detach().float() for b in self.biases])
+            if self.q is not None and self.q.device == w.device:
+                self._key = None
+                self._wait(w.device)         # (an earlier writing on another stream)
+                q, scale = quantize_fp8_weight(w.detach(), out=(self.q, self.scale))
+                b = self.b.copy_(b)
+            else:
+                q, scale = quantize_fp8_weight(w.detach())
+            stream = torch.cuda.current_stream(w.device)
+            written = torch.cuda.Event()
+            written.record(stream)
+        self.q, self.scale, self.b, self._written, self._stream, self._key = q, scale, b, written, stream.cuda_stream, key
 
     def __getstate__(self):
-        # a copied or pickled module writes copies of its own (an event can be neither)
-        return {**self.__dict__, "_key": None, "_written": None, "_stream": None, "q": None, "scale": None, "b": None}
+        # a copied or pickled module writes copies of its own (an event and a lock can be neither)
+        return {**self.__dict__, "_key": None, "_written": None, "_stream": None, "q": None, "scale": None, "b": None,
+                "_lock": None}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, _lock=threading.Lock())
 
     def _wait(self, device: torch.device) -> None:
         # (a capture begins behind a device synchronization, and must not wait for an event from outside it)

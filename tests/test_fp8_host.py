@@ -156,3 +156,53 @@ def test_fp32_product_refusals():
     assert gemm(ldc=7) == BADARG and gemm(lsa=1) == BADARG and gemm(lsb=1) == BADARG
     assert gemm(lda=264) == ALIGN and gemm(B=P + 8) == ALIGN and gemm(C=P + 2) == ALIGN and gemm(bias=P + 2) == ALIGN
     assert gemm(K=(1 << 28) + 1, lda=1 << 29, ldb=1 << 29, lsa=1 << 22, lsb=1 << 22) == SHAPE
+
+
+def test_copies_of_weights_are_written_by_one_thread(monkeypatch):
+    """Threads that find the copies stale together: one writes, the others wait for it and see values, scales, bias and event whole."""
+    import copy
+    import threading
+    import time
+    import types
+
+    from src import ops
+    writes = []
+
+    def quantize(w, out=None):
+        writes.append(threading.get_ident())
+        time.sleep(0.02)
+        return out or (torch.zeros(3, 4), torch.zeros(1, 1))
+
+    def event():
+        time.sleep(0.02)
+        return types.SimpleNamespace(record=lambda s: None)
+
+    def wait(self, device):
+        assert self._written is not None and self.b is not None and self._stream == 7
+
+    monkeypatch.setattr(ops, "quantize_fp8_weight", quantize)
+    monkeypatch.setattr(ops.Fp8Weights, "_wait", wait)
+    monkeypatch.setattr(torch.cuda, "Event", event)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: types.SimpleNamespace(cuda_stream=7))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    w, b = torch.nn.Parameter(torch.zeros(3, 4)), torch.nn.Parameter(torch.zeros(3))
+    pack = ops.Fp8Weights([w], [b])
+    for step in range(3):
+        got, failed = [], []
+
+        def call():
+            try:
+                got.append(pack.get())
+            except BaseException as e:
+                failed.append(e)
+        threads = [threading.Thread(target=call) for _ in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not failed and len(got) == 8 and len(writes) == step + 1, (failed, len(writes))
+        assert all(g[0] is got[0][0] and g[2] is not None for g in got)
+        with torch.no_grad():
+            w.add_(1.0)
+    twin = copy.deepcopy(pack)
+    assert twin.q is None and twin.get()[0] is not pack.get()[0]

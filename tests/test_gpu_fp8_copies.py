@@ -22,3 +22,36 @@ def test_copies_made_in_inference_mode_are_written_again_outside_it(dev):
         lin[3].bias.mul_(2.0)
     with torch.inference_mode():          # and the other way round
         assert torch.equal(ops.fp8_linear(x, packs[2]), 4 * y0)
+
+
+def test_threads_with_streams_of_their_own(dev):
+    import threading
+
+    from src import ops
+    lin, packs = make_layer(dev)
+    x = torch.randn(300, 192, device=dev).bfloat16()
+    with torch.no_grad():
+        want = ops.fp8_linear(x, packs[2])
+    for step in range(4):
+        torch.cuda.synchronize()
+        start, out, failed = threading.Barrier(4), [None] * 4, []
+
+        def call(i):
+            try:
+                with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                    start.wait()
+                    out[i] = ops.fp8_linear(x, packs[2])
+            except BaseException as e:
+                failed.append(e)
+        threads = [threading.Thread(target=call, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not failed, failed
+        assert all(torch.equal(y, want) for y in out)
+        with torch.no_grad():
+            lin[3].weight.mul_(2.0)
+            lin[3].bias.mul_(2.0)
+        want = 2 * want
