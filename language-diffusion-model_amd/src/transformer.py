@@ -79,6 +79,16 @@ class RMSNorm(nn.Module):
         return ops.rms_norm_with_residual(x, self.weight, self.eps, out_dtype)
 
 
+def _fp8_copies(packs: dict, which: str, lin) -> ops.Fp8Weights:
+    """packs[which], the 8-bit copies of the projections ``lin``; new ones where a parameter is another object than the one
+    they were made of (``load_state_dict(assign=True)``, an assigned ``weight``)."""
+    pack = packs.get(which)
+    weights, biases = [m.weight for m in lin], [m.bias for m in lin]
+    if pack is None or any(a is not b for a, b in zip(pack.weights + pack.biases, weights + biases)):
+        pack = packs[which] = ops.Fp8Weights(weights, biases)
+    return pack
+
+
 class SwiGLU(nn.Module):
     """w3( w1(x) * silu(w2(x)) ) -- the gate is w2 (src/transformer.py:91-95)."""
 
@@ -102,10 +112,7 @@ class SwiGLU(nn.Module):
         return self._packs[key]
 
     def _fp8_pack(self, which: str) -> ops.Fp8Weights:
-        if which not in self._fp8_packs:
-            lin = (self.w1, self.w2) if which == "in" else (self.w3,)
-            self._fp8_packs[which] = ops.Fp8Weights([m.weight for m in lin], [m.bias for m in lin])
-        return self._fp8_packs[which]
+        return _fp8_copies(self._fp8_packs, which, (self.w1, self.w2) if which == "in" else (self.w3,))
 
     def forward_fp8(self, x: tuple[Tensor, Tensor]) -> Tensor:
         """8-bit rows in, bf16 out (inference): gate/up product, 8-bit rows of ``a * silu(g)``, down product."""
@@ -212,10 +219,8 @@ class RotaryMultiheadAttention(nn.Module):
         return self._packs[key]
 
     def _fp8_pack(self, which: str) -> ops.Fp8Weights:
-        if which not in self._fp8_packs:
-            lin = (self.q_proj, self.k_proj, self.v_proj) if which == "qkv" else (self.out_proj,)
-            self._fp8_packs[which] = ops.Fp8Weights([m.weight for m in lin], [m.bias for m in lin])
-        return self._fp8_packs[which]
+        return _fp8_copies(self._fp8_packs, which,
+                           (self.q_proj, self.k_proj, self.v_proj) if which == "qkv" else (self.out_proj,))
 
     def forward_fp8(self, x: tuple[Tensor, Tensor], key_valid: Tensor | None) -> Tensor:
         """8-bit rows [B, S, d] in, bf16 out (inference): the projections in 8 bits, the attention itself in bf16."""
@@ -375,9 +380,7 @@ class DiffusionTransformer(nn.Module):
         return self._packs[key]
 
     def _fp8_head_pack(self) -> ops.Fp8Weights:
-        if "head" not in self._fp8_packs:
-            self._fp8_packs["head"] = ops.Fp8Weights([self.output_layer.weight], [self.output_layer.bias])
-        return self._fp8_packs["head"]
+        return _fp8_copies(self._fp8_packs, "head", (self.output_layer,))
 
     def _fp8_now(self) -> bool:
         """Whether this forward takes the 8-bit inference path."""

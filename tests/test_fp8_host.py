@@ -206,3 +206,23 @@ def test_copies_of_weights_are_written_by_one_thread(monkeypatch):
             w.add_(1.0)
     twin = copy.deepcopy(pack)
     assert twin.q is None and twin.get()[0] is not pack.get()[0]
+
+
+def test_copies_are_of_the_parameters_that_the_modules_hold_now():
+    from src.transformer import DiffusionTransformer, DiffusionTransformerConfig
+    cfg = DiffusionTransformerConfig(vocab_size=40, d_model=32, nhead=2, num_layers=1, dim_feedforward=24)
+    tr, other = DiffusionTransformer(cfg), DiffusionTransformer(cfg)
+    layer = tr.layers[0]
+
+    def packs():
+        return [layer.self_attn._fp8_pack("qkv"), layer.self_attn._fp8_pack("out"), layer.swiglu._fp8_pack("in"),
+                layer.swiglu._fp8_pack("out"), tr._fp8_head_pack()]
+    before = packs()
+    assert all(a is b for a, b in zip(before, packs()))
+    tr.load_state_dict(other.state_dict(), assign=True)
+    assert all(a is not b for a, b in zip(before, packs()))
+    held = {id(p) for p in tr.parameters()}
+    assert all(id(p) in held for pack in packs() for p in pack.weights + pack.biases)
+    layer.swiglu.w3.bias = torch.nn.Parameter(torch.ones(32))
+    now = packs()
+    assert now[3].biases[0] is layer.swiglu.w3.bias and now[2] is packs()[2]

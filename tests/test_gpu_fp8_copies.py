@@ -55,3 +55,15 @@ def test_threads_with_streams_of_their_own(dev):
             lin[3].weight.mul_(2.0)
             lin[3].bias.mul_(2.0)
         want = 2 * want
+
+
+@torch.no_grad()
+def test_parameters_replaced_by_others(dev):
+    tr, other = make(dev, fp8_head=True).eval().transformer, make(dev, fp8_head=True).eval().transformer
+    for p in other.parameters():
+        p.add_(0.01 * torch.randn_like(p))
+    ids, att = batch(dev)
+    tr(ids, att)
+    want = other(ids, att)
+    tr.load_state_dict(other.state_dict(), assign=True)
+    assert torch.equal(tr(ids, att), want)
