@@ -13,6 +13,7 @@ import threading
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _native as N
 
@@ -1344,11 +1345,15 @@ E8M0 = torch.float8_e8m0fnu     # power-of-two scales
 
 def _inference_inputs(what: str, first: Tensor, *others, differentiable: bool = True) -> torch.device:
     """The ROCm device all tensors (None: absent) share.  Raises for host tensors, mixed devices, and (where the result
-    would have one) tensors that need a gradient."""
+    would have one) tensors that need a gradient or carry a tangent of forward-mode differentiation."""
     dev = first.device
     grad = differentiable and torch.is_grad_enabled()
     if grad and first.requires_grad:
         raise RuntimeError(_NO_GRADIENT.format(what))
+    if differentiable and _forward_ad._current_level >= 0:      # (inside dual_level)
+        for t in (first, *others):
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} is an inference operator and has no derivative: a tensor with a tangent was given")
     if not first.is_cuda:
         N.require_device(first)
     for t in others:

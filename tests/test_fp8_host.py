@@ -226,3 +226,24 @@ def test_copies_are_of_the_parameters_that_the_modules_hold_now():
     layer.swiglu.w3.bias = torch.nn.Parameter(torch.ones(32))
     now = packs()
     assert now[3].biases[0] is layer.swiglu.w3.bias and now[2] is packs()[2]
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation: a tensor with a tangent would lose it without a word."""
+    from torch.autograd import forward_ad
+
+    from src import ops
+    x, w = torch.ones(4, 8), torch.ones(8)
+    q = torch.zeros(4, 16).to(torch.float8_e4m3fn)
+    s = torch.zeros(4, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    with forward_ad.dual_level():
+        dual, dw = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: ops.quantize_fp8(dual), lambda: ops.quantize_fp8(dual, "swiglu"),
+                     lambda: ops.rms_norm_fp8(dual, w, 1e-6), lambda: ops.rms_norm_fp8(x, dw, 1e-6),
+                     lambda: ops.rms_norm_fp8(x, w, 1e-6, residual=dual),
+                     lambda: ops.fp8_matmul(q[:, :8], s, q[:, :8], s[:1], bias=forward_ad.make_dual(torch.ones(4), torch.ones(4)))):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent|ROCm device") as e:
+                call()
+            assert "tangent" in str(e.value)
+        with pytest.raises(RuntimeError, match="ROCm device"):      # tensors without one: as ever
+            ops.quantize_fp8(x)
