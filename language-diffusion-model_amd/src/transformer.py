@@ -468,6 +468,11 @@ class DiffusionTransformer(nn.Module):
         from .loss import variational_lower_bound_loss
         if normalize_by not in ("masked", "tokens"):
             raise ValueError(f"normalize_by must be 'masked' or 'tokens', got {normalize_by!r}")
+        if self.fp8_head and self._fp8_now():      # (the fused head loss has no 8-bit form)
+            return variational_lower_bound_loss(logits=self.forward(masked_input_ids, attention_mask), targets=targets,
+                                                masked_input_ids=masked_input_ids, mask_token_id=mask_token_id,
+                                                attention_mask=attention_mask, seq_weight=seq_weight,
+                                                normalize_by=normalize_by)
         x = self.hidden_states(masked_input_ids, attention_mask)
         pack = self._head_pack()
         x2 = x.reshape(-1, x.shape[-1])
