@@ -87,6 +87,10 @@ __global__ __launch_bounds__(256) void rmsnorm_fp8_k(NormArgs a) {
     const unsigned code = fp8_scale_code(m);
     const float inv = fp8_inv_scale(code);
     if (c < a.d) {
+      if (c + 8 > a.d) {      // (zeros behind the last column: 0 * rstd is NaN in a row with a NaN)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = c + j < a.d ? v[i][j] : 0.f;
+      }
       uint2 p;
       p.x = fp8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
       p.y = fp8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
