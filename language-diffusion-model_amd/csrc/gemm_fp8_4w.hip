@@ -426,7 +426,8 @@ int ldm_gemm_fp8_4w(int64_t M, int64_t N, int64_t K, const uint8_t *A, int64_t l
   if (lda % 16 || ldb % 16 || ldc % 8 || !aligned_to(A, 16) || !aligned_to(B, 16) || !aligned_to(C, 16) ||
       (bias && !aligned_to(bias, 16)))
     return LDM_E_ALIGN;
-  // 32-bit lane offsets: 16 rows of an operand plus the k offset, 128 rows of C
+  // Lane offsets are unsigned 32-bit: up to 15 rows of A and 39 of B (src_b) plus K <= ldb, 40 x 2^26 < 2^32; 128 rows of C
+  // (2 ldc bytes each), 2^31
   if (lda >= (1 << 26) || ldb >= (1 << 26) || ldc >= (1 << 23)) return LDM_E_SHAPE;
   const int64_t tm = ceil_div(M, 256), tn = ceil_div(N, 256);
   if (M > 0x7fffff00 || N > 0x7fffff00 || tm * tn > 0x3fffffff) return LDM_E_SHAPE;
