@@ -325,7 +325,7 @@ int ldm_quant_fp8_block(const float *w, int64_t ld_w, int64_t N, int64_t K, uint
 /* C[M, N] = sum over 128-column blocks of 2^(eA + eB) * A_block B_block^T (+ bias[N]): A [M, K] 8-bit rows with sA
  * [M, ceil(K / 128)], B [N, K] 8-bit weights with sB [ceil(N / 128), ceil(K / 128)], fp32 accumulation, C bf16.  Of eight
  * consecutive products the matrix unit drops what lies 2^-13 below the leading bit of the largest.
- * Any M, N, K; lda and ldb multiples of 16, A and B 16-byte aligned (LDM_E_ALIGN), every row readable to the next
+ * Any M, N, K whose output is at most 2^24 - 1 tiles of 64 x 128 (LDM_E_SHAPE); lda and ldb multiples of 16, A and B 16-byte aligned (LDM_E_ALIGN), every row readable to the next
  * multiple of 16 bytes (what lies beyond K does not matter). */
 int ldm_gemm_fp8(int64_t M, int64_t N, int64_t K, const uint8_t *A, int64_t lda, const uint8_t *sA, int64_t ld_sa,
                  const uint8_t *B, int64_t ldb, const uint8_t *sB, int64_t ld_sb, const float *bias, void *C,

@@ -198,7 +198,9 @@ int launch_norm(const NormArgs &a, hipStream_t s) {
   return LDM_OK;
 }
 
-bool fits_grid(int64_t blocks) { return blocks <= 0x7fffffff; }
+// Rows (or 128-column blocks of rows) of a launch: a grid of 2^32 threads and more is cut off without an error, so longer
+// inputs take several launches
+constexpr int64_t ROWS = 1 << 23, BLOCKS = 1 << 27;
 
 }  // namespace
 
@@ -209,17 +211,24 @@ extern "C" int ldm_rmsnorm_fp8(const void *x, int x_dtype, int64_t ld_x, const v
   if ((x_dtype != LDM_F32 && x_dtype != LDM_BF16) || (res && stream_dtype != LDM_F32 && stream_dtype != LDM_BF16))
     return LDM_E_DTYPE;
   if (res && x_dtype == LDM_F32 && stream_dtype == LDM_BF16) return LDM_E_DTYPE;
-  if (d > 16384) return LDM_E_SHAPE;
+  if (d > 16384 || T >= (1ll << 40)) return LDM_E_SHAPE;
   if (T == 0) return LDM_OK;
   if (!x || !w || !q || !scale || (res && !stream_out)) return LDM_E_BADARG;
   if (ld_x < d || (res && ld_res < d) || ld_s < ceil_div(d, FP8_BLOCK)) return LDM_E_BADARG;
   if (ld_q % 8 || ld_q < ceil_div(d, 8) * 8 || !aligned_to(q, 8)) return LDM_E_ALIGN;
-  if (!fits_grid(T)) return LDM_E_SHAPE;
-  NormArgs a{x, ld_x, res, ld_res, w, T, (int)d, eps, stream_out, q, ld_q, scale, ld_s};
   hipStream_t s = (hipStream_t)stream;
-  if (!res) return x_dtype == LDM_F32 ? launch_norm<float, float, false>(a, s) : launch_norm<bf16_t, bf16_t, false>(a, s);
-  if (x_dtype == LDM_F32) return launch_norm<float, float, true>(a, s);
-  return stream_dtype == LDM_F32 ? launch_norm<bf16_t, float, true>(a, s) : launch_norm<bf16_t, bf16_t, true>(a, s);
+  const int64_t xb = x_dtype == LDM_F32 ? 4 : 2, rb = stream_dtype == LDM_F32 ? 4 : 2;
+  for (int64_t t = 0; t < T; t += ROWS) {
+    const NormArgs a{(const char *)x + t * ld_x * xb, ld_x, res ? (const char *)res + t * ld_res * rb : nullptr, ld_res, w,
+                     T - t < ROWS ? T - t : ROWS, (int)d, eps, res ? (char *)stream_out + t * d * rb : nullptr,
+                     q + t * ld_q, ld_q, scale + t * ld_s, ld_s};
+    int rc;
+    if (!res) rc = x_dtype == LDM_F32 ? launch_norm<float, float, false>(a, s) : launch_norm<bf16_t, bf16_t, false>(a, s);
+    else if (x_dtype == LDM_F32) rc = launch_norm<float, float, true>(a, s);
+    else rc = stream_dtype == LDM_F32 ? launch_norm<bf16_t, float, true>(a, s) : launch_norm<bf16_t, bf16_t, true>(a, s);
+    if (rc != LDM_OK) return rc;
+  }
+  return LDM_OK;
 }
 
 extern "C" int ldm_quant_fp8(const void *x, int dtype, int64_t ld_x, int64_t T, int64_t d, int swiglu, uint8_t *q,
@@ -232,18 +241,22 @@ extern "C" int ldm_quant_fp8(const void *x, int dtype, int64_t ld_x, int64_t T, 
   const int64_t nb = ceil_div(d, FP8_BLOCK);
   if (ld_x < (swiglu ? 2 * d : d) || ld_s < nb) return LDM_E_BADARG;
   if (ld_q % 8 || ld_q < ceil_div(d, 8) * 8 || !aligned_to(q, 8)) return LDM_E_ALIGN;
-  if (T > INT64_MAX / nb || !fits_grid(ceil_div(T * nb, 16))) return LDM_E_SHAPE;
-  QuantArgs a{x, ld_x, T, (int)d, (int)nb, q, ld_q, scale, ld_s};
-  const dim3 grid((unsigned)ceil_div(T * nb, 16)), wg(256);
+  if (T >= (1ll << 40)) return LDM_E_SHAPE;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == LDM_F32) {
-    if (swiglu) hipLaunchKernelGGL((quant_fp8_k<float, true>), grid, wg, 0, s, a);
-    else hipLaunchKernelGGL((quant_fp8_k<float, false>), grid, wg, 0, s, a);
-  } else {
-    if (swiglu) hipLaunchKernelGGL((quant_fp8_k<bf16_t, true>), grid, wg, 0, s, a);
-    else hipLaunchKernelGGL((quant_fp8_k<bf16_t, false>), grid, wg, 0, s, a);
+  const int64_t most = BLOCKS / nb, xb = dtype == LDM_F32 ? 4 : 2;      // (nb <= 2^21)
+  for (int64_t t = 0; t < T; t += most) {
+    const int64_t rows = T - t < most ? T - t : most;
+    const QuantArgs a{(const char *)x + t * ld_x * xb, ld_x, rows, (int)d, (int)nb, q + t * ld_q, ld_q, scale + t * ld_s, ld_s};
+    const dim3 grid((unsigned)ceil_div(rows * nb, 16)), wg(256);
+    if (dtype == LDM_F32) {
+      if (swiglu) hipLaunchKernelGGL((quant_fp8_k<float, true>), grid, wg, 0, s, a);
+      else hipLaunchKernelGGL((quant_fp8_k<float, false>), grid, wg, 0, s, a);
+    } else {
+      if (swiglu) hipLaunchKernelGGL((quant_fp8_k<bf16_t, true>), grid, wg, 0, s, a);
+      else hipLaunchKernelGGL((quant_fp8_k<bf16_t, false>), grid, wg, 0, s, a);
+    }
+    LDM_CHECK_LAUNCH();
   }
-  LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
 

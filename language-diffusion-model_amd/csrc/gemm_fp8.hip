@@ -428,11 +428,14 @@ __global__ __launch_bounds__(256, 2) void gemm_fp8_tile_k(GArgs g, int tiles_m, 
   }
 }
 
+// workgroups along x: a grid of 2^32 threads and more is cut off without an error
+constexpr int64_t MAX_WGS = 0xffffffffll / 256;
+
 template <int TM, typename OT>
 int launch_tile(const GArgs &g, hipStream_t s) {
   constexpr int BM = 32 * TM, LDS = 2 * (BM + 128) * FP8_BLOCK + SCH * (BM + 1);
   const int64_t tm = ceil_div(g.M, BM), tn = ceil_div(g.N, 128);
-  if (tm > 0x3fffffff || tn > 0x3fffffff || tm * tn > 0x3fffffff) return LDM_E_SHAPE;
+  if (tm > MAX_WGS || tn > MAX_WGS || tm * tn > MAX_WGS) return LDM_E_SHAPE;
   // 32-bit source offsets inside a tile
   if (g.lda >= (1 << 23) || g.ldb >= (1 << 23)) return LDM_E_SHAPE;
   const bool vec = g.ldc % (16 / (int)sizeof(OT)) == 0 && aligned_to(g.C, 16);
@@ -453,7 +456,7 @@ int launch_rows(const GArgs &g, hipStream_t s) {
   const int64_t gx = ceil_div(g.N, 16);
   const int mt = g.M <= 16 ? 1 : g.M <= 32 ? 2 : 4;
   const int64_t gy = ceil_div(g.M, 16 * mt);
-  if (gx > 0x7fffffff || gy > 65535) return LDM_E_SHAPE;
+  if (gx > MAX_WGS || gy > 65535) return LDM_E_SHAPE;
   const dim3 grid((unsigned)gx, (unsigned)gy), wg(256);
   if (mt == 1) hipLaunchKernelGGL((gemm_fp8_rows_k<1, OT>), grid, wg, 0, s, g, vec);
   else if (mt == 2) hipLaunchKernelGGL((gemm_fp8_rows_k<2, OT>), grid, wg, 0, s, g, vec);

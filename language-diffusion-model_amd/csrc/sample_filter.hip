@@ -857,5 +857,17 @@ extern "C" int ldm_sample_filtered(const void *logits, int dtype, int64_t T, int
   a.shift = 62 - bits < 45 ? 62 - bits : 45;
   a.out = out;
   hipStream_t s = (hipStream_t)stream;
-  return dtype == LDM_F32 ? launch_rows<float>(logits, a, T, s) : launch_rows<bf16_t>(logits, a, T, s);
+  // (a grid of 2^32 threads and more is cut off without an error: longer inputs take several launches)
+  constexpr int64_t ROWS = 1 << 21;
+  for (int64_t t = 0; t < T; t += ROWS) {
+    const int64_t rows = T - t < ROWS ? T - t : ROWS;
+    FArgs b = a;
+    b.u += t;
+    if (b.ids) b.ids += t;
+    b.out += t;
+    const int rc = dtype == LDM_F32 ? launch_rows<float>((const float *)logits + t * ld, b, rows, s)
+                                    : launch_rows<bf16_t>((const bf16_t *)logits + t * ld, b, rows, s);
+    if (rc != LDM_OK) return rc;
+  }
+  return LDM_OK;
 }

@@ -247,3 +247,11 @@ def test_tangents_are_refused():
             assert "tangent" in str(e.value)
         with pytest.raises(RuntimeError, match="ROCm device"):      # tensors without one: as ever
             ops.quantize_fp8(x)
+
+
+def test_products_beyond_the_largest_grid_are_refused():
+    from src import _native as N
+    P = 4096      # an address that is never read
+    for entry in (N.lib().ldm_gemm_fp8, N.lib().ldm_gemm_fp8_f32):
+        for M, n in ((1, 1 << 29), (1 << 31, 1)):
+            assert entry(M, n, 16, P, 16, P, 1, P, 16, P, 1, None, P, n, None) == SHAPE
