@@ -79,9 +79,11 @@ class RMSNorm(nn.Module):
         return ops.rms_norm_with_residual(x, self.weight, self.eps, out_dtype)
 
 
-def _fp8_copies(packs: dict, which: str, lin) -> ops.Fp8Weights:
-    """packs[which], the 8-bit copies of the projections ``lin``; new ones where a parameter is another object than the one
-    they were made of (``load_state_dict(assign=True)``, an assigned ``weight``)."""
+def _fp8_copies(module: nn.Module, which: str, lin) -> ops.Fp8Weights:
+    """The 8-bit copies of ``module``'s projections ``lin``; new ones where a parameter is another object than the one they
+    were made of (``load_state_dict(assign=True)``, an assigned ``weight``)."""
+    # (not in _packs, which the optimizer refreshes; a module pickled by an earlier version has none)
+    packs = module.__dict__.setdefault("_fp8_packs", {})
     pack = packs.get(which)
     weights, biases = [m.weight for m in lin], [m.bias for m in lin]
     if pack is None or any(a is not b for a, b in zip(pack.weights + pack.biases, weights + biases)):
@@ -112,7 +114,7 @@ class SwiGLU(nn.Module):
         return self._packs[key]
 
     def _fp8_pack(self, which: str) -> ops.Fp8Weights:
-        return _fp8_copies(self._fp8_packs, which, (self.w1, self.w2) if which == "in" else (self.w3,))
+        return _fp8_copies(self, which, (self.w1, self.w2) if which == "in" else (self.w3,))
 
     def forward_fp8(self, x: tuple[Tensor, Tensor]) -> Tensor:
         """8-bit rows in, bf16 out (inference): gate/up product, 8-bit rows of ``a * silu(g)``, down product."""
@@ -219,7 +221,7 @@ class RotaryMultiheadAttention(nn.Module):
         return self._packs[key]
 
     def _fp8_pack(self, which: str) -> ops.Fp8Weights:
-        return _fp8_copies(self._fp8_packs, which,
+        return _fp8_copies(self, which,
                            (self.q_proj, self.k_proj, self.v_proj) if which == "qkv" else (self.out_proj,))
 
     def forward_fp8(self, x: tuple[Tensor, Tensor], key_valid: Tensor | None) -> Tensor:
@@ -350,11 +352,14 @@ class DiffusionTransformer(nn.Module):
         # bf16 deviation on single deep-layer gradient tensors, while loss and whole gradient stay within 2e-2.
         # The fp32 stream runs its additions and casts as separate passes.
         self.fp32_residual = False
-        # True (with the bf16 compute dtype): forwards without gradients and without active dropout -- generate, sample,
-        # evaluate -- run the layers' projections in 8 bits (e4m3, power-of-two scales per 128 columns / 128 x 128 block
-        # of the weights); attention, norms and the residual stream stay as they are.  fp8_head: the LM head as well.
-        self.fp8_inference = False
-        self.fp8_head = False
+
+    # True (with the bf16 compute dtype): forwards without gradients and without active dropout -- generate, sample,
+    # evaluate -- run the layers' projections in 8 bits (e4m3, power-of-two scales per 128 columns / 128 x 128 block
+    # of the weights); attention, norms and the residual stream stay as they are.  fp8_head: the LM head as well.
+    # Such a forward calls the operators itself: forward hooks and replaced ``forward`` methods of the layers, norms,
+    # attention and SwiGLU modules do not run in it.  (On the class, for models pickled by an earlier version.)
+    fp8_inference: bool = False
+    fp8_head: bool = False
 
     def _init_parameters(self) -> None:
         """Xavier-uniform on every parameter with dim() > 1 (src/transformer.py:407-411)."""
@@ -380,7 +385,7 @@ class DiffusionTransformer(nn.Module):
         return self._packs[key]
 
     def _fp8_head_pack(self) -> ops.Fp8Weights:
-        return _fp8_copies(self._fp8_packs, "head", (self.output_layer,))
+        return _fp8_copies(self, "head", (self.output_layer,))
 
     def _fp8_now(self) -> bool:
         """Whether this forward takes the 8-bit inference path."""

@@ -255,3 +255,24 @@ def test_products_beyond_the_largest_grid_are_refused():
     for entry in (N.lib().ldm_gemm_fp8, N.lib().ldm_gemm_fp8_f32):
         for M, n in ((1, 1 << 29), (1 << 31, 1)):
             assert entry(M, n, 16, P, 16, P, 1, P, 16, P, 1, None, P, n, None) == SHAPE
+
+
+def test_models_pickled_before_the_8_bit_path():
+    """Their objects have none of its attributes: off by default, and usable."""
+    import pickle
+
+    from src.transformer import DiffusionTransformer, DiffusionTransformerConfig
+    tr = DiffusionTransformer(DiffusionTransformerConfig(vocab_size=40, d_model=32, nhead=2, num_layers=1, dim_feedforward=24))
+    for m in tr.modules():
+        for name in ("_fp8_packs", "fp8_inference", "fp8_head"):
+            m.__dict__.pop(name, None)
+    tr = pickle.loads(pickle.dumps(tr))
+    with torch.no_grad():
+        assert tr._fp8_now() is False and tr.fp8_head is False
+    layer = tr.layers[0]
+    assert tr._fp8_head_pack() is tr._fp8_head_pack()
+    assert layer.self_attn._fp8_pack("qkv") is layer.self_attn._fp8_pack("qkv") is not layer.self_attn._fp8_pack("out")
+    assert layer.swiglu._fp8_pack("in").weights[1] is layer.swiglu.w2.weight
+    other = DiffusionTransformer(DiffusionTransformerConfig(vocab_size=40, d_model=32, nhead=2, num_layers=1, dim_feedforward=24))
+    other.fp8_inference = True
+    assert tr.fp8_inference is False and other.layers[0].swiglu._fp8_pack("in") is not layer.swiglu._fp8_pack("in")
