@@ -1580,7 +1580,8 @@ class Fp8Weights:
     """8-bit copies of projections that share an input (the inference twin of PackedWeights): values, block scales and
     fp32 bias, written again, in place, by ``get()`` when a parameter changed.  A stream other than the one that wrote
     them waits for that.  They are not written while a graph is captured (nothing would run, and every replay would write
-    them again): call the projection once before the capture; a captured graph reads what the last eager ``get()`` left."""
+    them again): call the projection once before the capture; a captured graph reads what the last eager ``get()`` left, and a
+    replay on another stream than that call's has to be ordered behind it, as for every tensor that a graph reads."""
 
     def __init__(self, weights, biases):
         self.weights = list(weights)
