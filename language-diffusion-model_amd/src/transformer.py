@@ -405,6 +405,12 @@ class DiffusionTransformer(nn.Module):
             branch, stream = layer.forward_fp8(branch, stream, key_valid)
         return branch, stream
 
+    def _fp8_logits(self, input_ids: Tensor, attention_mask: Tensor | None) -> Tensor:
+        """The bf16 logits with layers and head in 8 bits."""
+        branch, stream = self._fp8_layers(input_ids, attention_mask)
+        q, s, _ = ops.rms_norm_fp8(branch, self.norm.weight, self.norm.eps, residual=stream)
+        return ops.fp8_linear((q, s), self._fp8_head_pack())
+
     def hidden_states(self, input_ids: Tensor, attention_mask: Tensor | None = None) -> Tensor:
         """Everything of forward() up to and including the final norm: [B,S,d]."""
         if self._fp8_now():
@@ -453,9 +459,7 @@ class DiffusionTransformer(nn.Module):
         The logits rows are stored with a stride padded to 64 columns; the returned
         tensor is the [B,S,V] view of that buffer."""
         if self.fp8_head and self._fp8_now():
-            branch, stream = self._fp8_layers(input_ids, attention_mask)
-            q, s, _ = ops.rms_norm_fp8(branch, self.norm.weight, self.norm.eps, residual=stream)
-            logits = ops.fp8_linear((q, s), self._fp8_head_pack())
+            logits = self._fp8_logits(input_ids, attention_mask)
         else:
             logits = ops.packed_linear(self.hidden_states(input_ids, attention_mask), self._head_pack())
         if self.fp32_logits and logits.dtype != torch.float32:
@@ -474,7 +478,7 @@ class DiffusionTransformer(nn.Module):
         if normalize_by not in ("masked", "tokens"):
             raise ValueError(f"normalize_by must be 'masked' or 'tokens', got {normalize_by!r}")
         if self.fp8_head and self._fp8_now():      # (the fused head loss has no 8-bit form)
-            return variational_lower_bound_loss(logits=self.forward(masked_input_ids, attention_mask), targets=targets,
+            return variational_lower_bound_loss(logits=self._fp8_logits(masked_input_ids, attention_mask), targets=targets,
                                                 masked_input_ids=masked_input_ids, mask_token_id=mask_token_id,
                                                 attention_mask=attention_mask, seq_weight=seq_weight,
                                                 normalize_by=normalize_by)

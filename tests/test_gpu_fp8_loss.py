@@ -24,6 +24,9 @@ def test_loss_without_gradients_is_that_of_the_logits(dev, kw, fp32_residual):
     got = tr.masked_token_loss(ids, targets, 103, att, **kw)
     want = variational_lower_bound_loss(logits=tr(ids, att), targets=targets, masked_input_ids=ids, mask_token_id=103,
                                         attention_mask=att, **kw)
+    tr.fp32_logits = True      # (the same values, widened)
+    assert tr(ids, att).dtype == torch.float32
+    assert abs(float(tr.masked_token_loss(ids, targets, 103, att, **kw)) - float(want)) <= 40 * 2.0 ** -24 * abs(float(want))
     # (fp32 sums of at most 40 masked rows' losses, all of one sign, maybe in another order)
     assert abs(float(got) - float(want)) <= 40 * 2.0 ** -24 * abs(float(want))
     tr.fp8_head = False
